@@ -1,0 +1,38 @@
+"""The scripts of scripts/: what may be in them, and that the documents name only those that are there.
+
+A build whose kernels fault or hang on the GPU is not run there again to narrow the failure down: the cause is looked for on the CPU (tests/wavemu executes the kernel source,
+tests/isaemu the kernel binary).  So no GPU script may be one that does it."""
+import glob
+import os
+import re
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+FOLDERS = [os.path.join(ROOT, "scripts", d) for d in ("", "archive", "calib")]
+GPU_SCRIPTS = sorted(p for d in FOLDERS for p in glob.glob(os.path.join(d, "gpu_*")))
+DOCUMENTS = [os.path.join(ROOT, f) for f in ("README.md", "DESIGN.md", "INTEGRATION.md")] + sorted(glob.glob(os.path.join(ROOT, "profiles", "*.md")) + glob.glob(os.path.join(ROOT, "profiles", "*.txt")))
+FAULT_WORDS = re.compile(r"\b(faults?|faulted|faulting|aborts?|aborted|hangs?|hung|crash\w*)\b", re.I)
+FAILED_BUILDS = re.compile(r"libhpt_(prodfail|debugra|noslp|nosv|wait0|cw3|runB)\b|Memory access fault")
+
+
+def explanations(text):
+    """the comment lines and the docstring of a script"""
+    doc = re.findall(r'"""(.*?)"""', text, re.S)
+    return "\n".join([l for l in text.splitlines() if l.lstrip().startswith("#")] + doc)
+
+
+@pytest.mark.parametrize("path", GPU_SCRIPTS, ids=os.path.basename)
+def test_no_gpu_script_is_there_to_make_a_failure_happen_again(path):
+    text = open(path).read()
+    assert not FAULT_WORDS.search(explanations(text)), explanations(text)
+    assert not FAILED_BUILDS.search(text)
+
+
+def test_documents_name_only_scripts_that_are_in_the_tree():
+    missing = set()
+    for doc in DOCUMENTS:
+        for name in re.findall(r"scripts/[\w./]+?\.(?:sh|py|hip|cpp)\b|\bgpu_\w+\.(?:sh|py)\b", open(doc, errors="replace").read()):
+            if not any(os.path.exists(os.path.join(d, os.path.basename(name))) for d in FOLDERS):
+                missing.add((os.path.relpath(doc, ROOT), name))
+    assert not missing, sorted(missing)
