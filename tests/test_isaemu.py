@@ -153,6 +153,25 @@ def test_shipped_kernel_binaries_render_the_oracles_film_in_the_interpreter(unit
     assert rmse < 1e-5 and off == 0, (rmse, off)
 
 
+@needs_build
+def test_the_animated_reflection_scenes_kernel_renders_the_oracles_film_in_the_interpreter():
+    """scenes/anim-moving-reflection.pbrt (an animated textured sphere over a mirror, direct lighting): the direct-lighting kernel of the instanced full set, the one its
+    end-to-end test runs on the GPU, from the built object — the four corners and the centre of the 100 x 100 fixture"""
+    s = load_case("aquaddl")
+    symbol = R.kernel_symbol(False, True, 31, 3, 0, True, True, True)
+    render = R.BinaryRender(s, R.code_object_for("ext_i", symbol), symbol, w.K_DL)
+    for x, y in ((0, 0), (92, 0), (0, 92), (92, 92), (46, 46)):
+        rd = hash_rd(s, seed=0)
+        rd.x_start += x
+        rd.y_start += y
+        rd.x_count = rd.y_count = 8
+        fo, so = orc.OracleScene(s).render(s.camera, rd)
+        f, info = render.render(s.camera, rd)
+        rmse, off = compare(f, fo)
+        assert info["samples"] == int(so[0]) and info["bad"] == 0 and np.array_equal(f[..., 3], fo[..., 3]), (x, y)
+        assert rmse < 1e-5 and off == 0, (x, y, rmse, off)
+
+
 # ---- round 5's failure, reproduced and repaired on the CPU ------------------------------------------------------------------------------
 def test_the_failing_build_of_round_5_fails_in_the_interpreter_and_one_moved_instruction_repairs_it():
     """libhpt_prodfail.so (GPU run D of round 5: aquad and oinst wrong at configuration 6 — 9 035 of 10 000 pixels, 60 910 bad samples): its kernel, interpreted,

@@ -36,3 +36,11 @@ def test_documents_name_only_scripts_that_are_in_the_tree():
             if not any(os.path.exists(os.path.join(d, os.path.basename(name))) for d in FOLDERS):
                 missing.add((os.path.relpath(doc, ROOT), name))
     assert not missing, sorted(missing)
+
+
+@pytest.mark.parametrize("path", GPU_SCRIPTS, ids=os.path.basename)
+def test_no_gpu_script_repeats_a_test_to_see_whether_it_fails_again(path):
+    """passes of another build say nothing about the one that failed, and a loop that drops the exit status does not stop at the first failure"""
+    text = open(path).read()
+    for loop in re.findall(r"^for (?:i|rep) in [\d ]+; do(.*?)^done", text, re.S | re.M):
+        assert "pytest" not in loop, loop
