@@ -112,7 +112,7 @@ def parse_insn(addr, size, text):
     parts = text.split(None, 1)
     ins.op = parts[0]
     rest = " " + parts[1] if len(parts) > 1 else ""
-    if ins.op in ("s_waitcnt", "s_nop", "s_sleep", "s_setprio", "s_endpgm", "s_barrier", "s_waitcnt_depctr", "s_sethalt", "s_trap", "s_setreg_imm32_b32", "s_setreg_b32", "s_icache_inv", "s_dcache_wb",
+    if ins.op in ("s_waitcnt", "s_nop", "s_sleep", "s_setprio", "s_endpgm", "s_barrier", "s_waitcnt_depctr", "s_sethalt", "s_trap", "s_setreg_imm32_b32", "s_setreg_b32", "s_icache_inv",
                   "buffer_wbl2", "buffer_inv", "s_ttracedata", "s_code_end", "s_waitcnt_vscnt", "s_set_gpr_idx_off"):
         ins.ops = []
         return ins
@@ -694,8 +694,6 @@ def bind_scalar(ins):
             for j in range(n):
                 w.S[ops[0].idx + j] = a[j]
         return fl
-    if op in ("s_store_dword", "s_atomic_add"):
-        raise EmuError("scalar stores are not used by the path kernels")
     return None
 
 
@@ -1348,7 +1346,7 @@ def bind_memory(ins):
 
 def bind(ins):
     op = ins.op
-    if op in ("s_waitcnt", "s_nop", "s_sleep", "s_setprio", "s_barrier", "s_waitcnt_depctr", "s_icache_inv", "s_dcache_wb", "buffer_wbl2", "buffer_inv", "s_waitcnt_vscnt", "s_setreg_imm32_b32", "s_ttracedata"):
+    if op in ("s_waitcnt", "s_nop", "s_sleep", "s_setprio", "s_barrier", "s_waitcnt_depctr", "s_icache_inv", "buffer_wbl2", "buffer_inv", "s_waitcnt_vscnt", "s_setreg_imm32_b32", "s_ttracedata"):
         return _nop
     if op == "s_endpgm":
         return _endpgm

@@ -10,6 +10,7 @@ film.  scripts/check_exec_restore.py finds the shape in any build without runnin
 import ctypes as C
 import importlib
 import os
+import re
 import subprocess
 import sys
 
@@ -130,6 +131,20 @@ def test_interpreter_does_64_bit_integers_and_strided_global_memory(tmp_path):
         for j in range(K):
             acc[i] = np.float32(acc[i] + np.float32(col[K - 1 - j][(i * 5 + 1) & 63] * np.float32(j & 3)))
     assert np.array_equal(acc, out[:64])
+
+
+@pytest.mark.parametrize("text", ["s_no_such", "s_no_such s[0:1]", "s_no_such s2, s[0:1], 0x10", "v_no_such v0, v1", "global_no_such v0, v[2:3], off"])
+def test_interpreter_refuses_an_instruction_it_does_not_know(text):
+    ins = g.parse_insn(0, 8, text)
+    with pytest.raises(g.EmuError, match="not implemented"):
+        g.bind(ins)
+    assert list(g.unimplemented([ins])) == [text.split()[0]]
+
+
+def test_interpreter_knows_no_scalar_memory_operation_but_loads():
+    """the path kernels write through vector stores only: what goes through the scalar data cache the other way is refused like any unknown instruction, and its source names none of it"""
+    named = set(re.findall(r"\bs_\w*(?:load|store|atomic|cache)\w*", open(g.__file__).read()))
+    assert named == {"s_load_dword", "s_icache_inv"}, named
 
 
 # ---- the binaries the build ships, on the CPU ----------------------------------------------------------------------------------------------
