@@ -19,7 +19,6 @@ template <int KIND> __global__ __launch_bounds__(256) void k(float *out, int n, 
 #define MINU(i) asm volatile("v_min_u32 %0, %0, %1" : "+v"(ia[i]) : "v"(ib));
 #define BFE(i) asm volatile("v_bfe_u32 %0, %0, %1, 5" : "+v"(ia[i]) : "v"(ib));
 #define CMPSEL(i) asm volatile("v_cmp_lt_f32 vcc, %0, %1\n v_cndmask_b32 %0, %0, %2, vcc" : "+v"(a[i]) : "v"(b), "v"(c) : "vcc");
-#define PKFMA(i) asm volatile("v_pk_fma_f32 %0, %0, %1, %2" : "+v"(*(double *)&a[(i) & 14]) : "v"(*(double *)&a[14]), "v"(*(double *)&a[12]));
 #define RCP(i) asm volatile("v_rcp_f32 %0, %0" : "+v"(a[i]));
 #define SQRT(i) asm volatile("v_sqrt_f32 %0, %0" : "+v"(a[i]));
 #define FMA64(i) asm volatile("v_fma_f64 %0, %0, %1, %1" : "+v"(*(double *)&a[(i) & 14]) : "v"(*(double *)&a[14]));
@@ -45,7 +44,7 @@ template <int KIND> __global__ __launch_bounds__(256) void k(float *out, int n, 
 #define MULLO(i) asm volatile("v_mul_lo_u32 %0, %0, %1" : "+v"(ia[i]) : "v"(ib));
         if (KIND == 0) { REP16(FMA) } else if (KIND == 1) { REP16(MUL) } else if (KIND == 2) { REP16(ADDU) } else if (KIND == 3) { REP16(CVT) }
         else if (KIND == 4) { REP16(FLOOR) } else if (KIND == 5) { REP16(MINU) } else if (KIND == 6) { REP16(BFE) } else if (KIND == 7) { REP16(CMPSEL) }
-        else if (KIND == 8) { REP16(PKFMA) } else if (KIND == 9) { REP16(RCP) } else if (KIND == 10) { REP16(SQRT) } else if (KIND == 11) { REP16(FMA64) }
+        else if (KIND == 9) { REP16(RCP) } else if (KIND == 10) { REP16(SQRT) } else if (KIND == 11) { REP16(FMA64) }
         else if (KIND == 16) { REP16(MINF) } else if (KIND == 17) { REP16(MAX3) } else if (KIND == 18) { REP16(SUBF) } else if (KIND == 19) { REP16(FMAC) }
         else if (KIND == 20) { REP16(CNDM) } else if (KIND == 21) { REP16(CMP) } else if (KIND == 22) { REP16(MOV) } else if (KIND == 23) { REP16(XOR) }
         else if (KIND == 24) { REP16(LSHL) } else if (KIND == 25) { REP16(MUL64) } else if (KIND == 26) { REP16(ADD64) } else if (KIND == 27) { REP16(CVT64) }
@@ -71,7 +70,7 @@ int main() {
     for (int wps : {32}) {
         run<0>("v_fma_f32", wps, 16); run<1>("v_mul_f32", wps, 16); run<2>("v_add_u32", wps, 16); run<3>("v_cvt_i32_f32", wps, 16);
         run<4>("v_floor_f32", wps, 16); run<5>("v_min_u32", wps, 16); run<6>("v_bfe_u32", wps, 16); run<7>("v_cmp+v_cndmask", wps, 32);
-        run<8>("v_pk_fma_f32", wps, 16); run<9>("v_rcp_f32", wps, 16); run<10>("v_sqrt_f32", wps, 16); run<11>("v_fma_f64", wps, 16);
+        run<9>("v_rcp_f32", wps, 16); run<10>("v_sqrt_f32", wps, 16); run<11>("v_fma_f64", wps, 16);
         run<12>("v_lshl_add_u32", wps, 16); run<13>("v_and_b32", wps, 16); run<14>("v_mad_u32_u24", wps, 16); run<15>("v_mul_lo_u32", wps, 16);
         run<16>("v_min_f32", wps, 16); run<17>("v_max3_f32", wps, 16); run<18>("v_sub_f32", wps, 16); run<19>("v_fmac_f32", wps, 16);
         run<20>("v_cndmask_b32", wps, 16); run<21>("v_cmp_lt_f32", wps, 16); run<22>("v_mov_b32", wps, 16); run<23>("v_xor_b32", wps, 16);

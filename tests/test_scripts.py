@@ -29,6 +29,16 @@ def test_no_gpu_script_is_there_to_make_a_failure_happen_again(path):
     assert not FAILED_BUILDS.search(text)
 
 
+def test_no_source_writes_packed_fp32_arithmetic_by_hand():
+    """v_pk_add_f32 and its kind have given wrong results on the GPU now and then, without an error: no inline assembly issues them, in the product or beside it"""
+    sources = [p for d in ("pbrt-v2_amd/csrc", "scripts/calib", "tests/isaemu/battery") for p in glob.glob(os.path.join(ROOT, d, "*")) if os.path.isfile(p)]
+    assert len(sources) > 30
+    for path in sources:
+        for line in open(path, errors="replace"):
+            if "asm" in line or "scripts" in path:
+                assert not re.search(r"v_pk_(add|mul|fma)_f32", line), (path, line)
+
+
 def test_documents_name_only_scripts_that_are_in_the_tree():
     missing = set()
     for doc in DOCUMENTS:
