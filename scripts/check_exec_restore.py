@@ -30,6 +30,8 @@ BUNDLER = "/opt/rocm/lib/llvm/bin/clang-offload-bundler"
 OBJCOPY = "/opt/rocm/lib/llvm/bin/llvm-objcopy"
 EXEC_RESTORE = re.compile(r"^(s_or_b64 exec, exec, |s_or_saveexec_b64 |s_andn2_saveexec_b64 |s_xor_b64 exec, exec, |s_mov_b64 exec, |s_andn2_b64 exec, exec, |s_and_b64 exec, exec, |s_xor_saveexec_b64 |s_and_saveexec_b64 )")
 SCALAR_DEST_VALU = ("v_readlane_b32", "v_readfirstlane_b32", "v_cmp", "v_writelane_b32")
+SAVEEXEC = re.compile(r"^s_(and|andn2|or|xor)_saveexec_b64 (s\[\d+:\d+\]|vcc),")
+LONG_JUMP = re.compile(r"^s_getpc_b64 s\[(\d+):(\d+)\]; s_add_u32 s\1, s\1, (-?\w+); s_addc_u32 s\2, s\2, (-?\w+); s_setpc_b64 s\[\1:\2\]$")
 STOP = ("s_cbranch", "s_branch", "s_setpc", "s_swappc", "s_endpgm", "s_barrier")
 
 
@@ -107,21 +109,44 @@ def dest_vgprs(text):
     return {int(m.group(1))} if m else set()
 
 
+def skips_of(insns):
+    """where a wave goes when a block's lanes are none -> ([(index of the branch, target)] with the skipped block between them, [further targets]).
+    s_cbranch_execz names it.  s_cbranch_execnz names the block, entered with its lanes in EXEC, and what follows the branch is the skip: the code there, or, if the target is out of
+    a branch's reach, the long jump s_getpc_b64 / s_add_u32 / s_addc_u32 / s_setpc_b64.  (A branch on EXEC without a mask saved just above it ends a loop.)"""
+    skips, others = [], []
+    for i, (addr, text) in enumerate(insns):
+        if not text.startswith("s_cbranch_exec"):
+            continue
+        opens = any(SAVEEXEC.match(t) for _, t in insns[max(0, i - 3):i])
+        if text.startswith("s_cbranch_execz"):
+            off = int(text.split()[1])
+            if off < 32768:
+                skips.append((i, addr + 4 + 4 * off))
+            elif opens:
+                others.append(addr + 4 + 4 * (off - 65536))
+        elif opens and i + 1 < len(insns):
+            m = LONG_JUMP.match("; ".join(t for _, t in insns[i + 1:i + 5]))
+            if m:
+                dist = (int(m.group(3), 0) & 0xffffffff) | (int(m.group(4), 0) & 0xffffffff) << 32
+                if dist < 1 << 63:
+                    skips.append((i, insns[i + 1][0] + 4 + dist))
+                else:
+                    others.append(insns[i + 1][0] + 4 + dist - (1 << 64))
+            else:
+                others.append(insns[i + 1][0])
+    return skips, others
+
+
 def check_function(name, insns):
     """insns: [(addr, text)] of one function -> [(label addr, offending addr, offending text, restore addr, restore text)]
     The structure looked for is the compiler's own `if`: s_and_saveexec_b64 s[a:b], <cond> ; s_cbranch_execz L ; <then> ; L: ... ; s_or_b64 exec, exec, s[a:b]"""
     pos = {a: i for i, (a, t) in enumerate(insns)}
     found = []
-    for i, (addr, text) in enumerate(insns):
-        if not text.startswith("s_cbranch_execz"):
-            continue
-        off = int(text.split()[-1])
-        if off >= 32768:
-            continue                                  # (backward: a loop, not the skip of a `then` block)
-        label = addr + 4 + 4 * off
+    skips, others = skips_of(insns)
+    for i, label in skips:
         saved = None
         for a0, t0 in reversed(insns[max(0, i - 3):i]):
-            m = re.match(r"^s_(and|andn2|or|xor)_saveexec_b64 (s\[\d+:\d+\]|vcc),", t0)
+            m = SAVEEXEC.match(t0)
             if m:
                 saved = m.group(2)
                 break
@@ -148,13 +173,7 @@ def check_function(name, insns):
                 pending.append((a1, t1))
     # The same hazard at an `else`: the block that a skipped `then` lands in begins with the s_or_saveexec_b64 / s_andn2_saveexec_b64 that flips EXEC to the other lanes — a vector
     # register defined above it is defined for the wrong half of the wave.  (No build of rounds 4 / 5 has one; the shape is checked because it is the same mistake.)
-    targets = set()
-    for addr, text in insns:
-        if text.startswith(("s_cbranch_execz", "s_cbranch_execnz")):
-            off = int(text.split()[-1])
-            if off < 32768:
-                targets.add(addr + 4 + 4 * off)
-    for label in sorted(targets):
+    for label in sorted(set(label for _, label in skips) | set(others)):
         j = pos.get(label)
         if j is None:
             continue

@@ -219,6 +219,35 @@ def test_the_gate_finds_the_misplaced_copy_in_the_failing_build():
     assert [(f[2], f[3]) for f in defects] == [(0x92B9D0, "v_mov_b64_e32 v[150:151], v[10:11]")], found
 
 
+def listing(lines):
+    """(address, text) pairs of instructions of four bytes each -> an llvm-objdump listing"""
+    return ["0000000000000000 <k>:\n"] + ["\t%s // %012X: 00000000\n" % (text, 4 * i) for i, text in enumerate(lines)]
+
+
+LONG_JUMP = ["s_getpc_b64 s[98:99]", "s_add_u32 s98, s98, 0x%x", "s_addc_u32 s99, s99, 0", "s_setpc_b64 s[98:99]"]
+
+
+def test_the_gate_reads_a_skip_through_a_long_jump():
+    """a target out of a branch's reach: s_cbranch_execnz over a long jump.  The block behind the long jump runs with its lanes in EXEC, so its loads are its own business (the second
+    listing); the long jump's target is where the lanes that skipped arrive, so a load above the flip to them is the defect (the first), as it is behind a short branch (the third)"""
+    then_block = ["scratch_load_dword v0, off, off offset:8", "v_cmp_eq_u32_e32 vcc, 1, v0"]
+    flip = ["s_andn2_saveexec_b64 s[0:1], s[4:5]", "s_endpgm"]
+    jump = [t % (4 * 12 - 4 * 4) if "%" in t else t for t in LONG_JUMP]
+    enter = ["s_and_saveexec_b64 s[0:1], s[86:87]", "s_xor_b64 s[4:5], exec, s[0:1]"]
+    defects = lambda lines: [f[2:4] for f in gate.scan(listing(lines))[2] if f[-1].startswith("DEFINES")]   # noqa: E731
+    body = enter + ["s_cbranch_execnz 4"] + jump + ["v_mov_b32_e32 v9, 0"] * 5
+    assert defects(body + ["scratch_load_dword v0, off, off offset:4"] + flip) == [(48, "scratch_load_dword v0, off, off offset:4")]
+    assert defects(enter + ["s_cbranch_execnz 4"] + jump + then_block + flip) == []
+    assert defects(enter + ["s_cbranch_execz 2"] + ["v_mov_b32_e32 v9, 0"] * 2 + ["scratch_load_dword v0, off, off offset:4"] + flip) == [(20, "scratch_load_dword v0, off, off offset:4")]
+    # a block that two sites share: one enters it with s_cbranch_execnz and falls through to its own flip, the other skips it backwards, to that flip
+    shared = enter + ["s_cbranch_execnz 5"] + flip[:1] + ["s_endpgm"] + enter + ["s_cbranch_execz 65531"] + then_block + flip
+    assert defects(shared) == []
+    assert defects(enter + ["s_cbranch_execnz 6", "scratch_load_dword v0, off, off offset:4"] + shared[3:7] + ["s_cbranch_execz 65530"] + then_block + flip) == [(12, "scratch_load_dword v0, off, off offset:4")]
+    # the same at an `if` without an else: a definition above the restore that the block behind the long jump never writes
+    assert defects(["s_and_saveexec_b64 s[4:5], vcc", "v_nop"] + ["s_cbranch_execnz 4"] + jump + ["v_mov_b32_e32 v9, 0"] * 5 + ["v_mov_b32_e32 v1, v2", "s_or_b64 exec, exec, s[4:5]", "s_endpgm"]) \
+        == [(48, "v_mov_b32_e32 v1, v2")]
+
+
 # (the build that round 4's GPU runs validated had ONE site of this shape, in the free-running configuration 0 of the basic set; a barrier compiled into that instantiation only
 #  — hpt_kernels_impl.h, HPT_CODEGEN_NUDGE — removed it, every other kernel of the build stayed instruction for instruction the same: profiles/r05_isaemu_root_cause.md §4)
 @needs_build
