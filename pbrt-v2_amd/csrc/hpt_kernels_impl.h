@@ -674,8 +674,9 @@ __global__ __launch_bounds__(HPT_BLOCK, WAVES) void hpt_path_kernel(const PathKe
         // them).  A lane that has finished now WAITS — as a subtree thief in the walks — until regen_min lanes of the wave have finished,
         // or nobody else is left to wait for.
         // Lock step + stealing only (configurations 5 / 6 and direct lighting — what production runs): there a waiting lane works as a thief.
-        // (The free-running instantiation of the extension set with animated instances faulted under a threshold of 16 — GPU run B2 of round 4,
-        //  cause not found; the free-running and plain lock-step kernels keep the per-round flush they have always had.)
+        // (The free-running instantiation of the extension set with animated instances faulted with the batching compiled in; the same source renders the oracle's film on the CPU
+        //  scheduler, the fault is what the compiler's defect looks like when the register it misses is a pointer (profiles/r05_ab.md).  The free-running and plain lock-step kernels keep
+        //  the per-round flush they have always had.)
 #if defined(HPT_DEBUG_SHADOW) && defined(HPT_DEBUG_CHECKS)
         const bool keeps_ = lane.stage != ST_IDLE && !lane.fin;
 #endif
@@ -686,8 +687,6 @@ __global__ __launch_bounds__(HPT_BLOCK, WAVES) void hpt_path_kernel(const PathKe
         {
 #ifdef HPT_DBG_NO_REGEN
             const int regen_min = 1;
-#elif defined(HPT_REGEN_ALL)   /* (diagnostic build: the batching in EVERY kernel — the state of round 4's run B2, whose free-running instanced extension kernel faulted) */
-            const int regen_min = a.regen_min;
 #else
             const int regen_min = (STEAL && PHASED) ? a.regen_min : 1;
 #endif

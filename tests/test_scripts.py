@@ -29,6 +29,11 @@ def test_no_gpu_script_is_there_to_make_a_failure_happen_again(path):
     assert not FAILED_BUILDS.search(text)
 
 
+def test_no_switch_of_the_product_builds_a_kernel_that_is_known_to_fault():
+    for path in glob.glob(os.path.join(ROOT, "pbrt-v2_amd", "csrc", "*")) + [os.path.join(ROOT, "pbrt-v2_amd", "Makefile")]:
+        assert "HPT_REGEN_ALL" not in open(path).read(), path          # the batched refill in the free-running kernels
+
+
 def test_no_source_writes_packed_fp32_arithmetic_by_hand():
     """v_pk_add_f32 and its kind have given wrong results on the GPU now and then, without an error: no inline assembly issues them, in the product or beside it"""
     sources = [p for d in ("pbrt-v2_amd/csrc", "scripts/calib", "tests/isaemu/battery") for p in glob.glob(os.path.join(ROOT, d, "*")) if os.path.isfile(p)]
