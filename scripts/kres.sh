@@ -21,5 +21,5 @@ namespace hpt {
 template __global__ void hpt_path_kernel<false, K_INST, K_MATS, K_WAVES, 0, true, K_DL, true>(const PathKernelArgs a);
 }
 EOT
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-function -munsafe-fp-atomics -Icsrc \
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-function -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -Icsrc \
   -Rpass-analysis=kernel-resource-usage "$@" -c /tmp/k/one.hip -o /tmp/k/one.o 2>&1 | grep -E 'Function Name|VGPRs:|ScratchSize|Occupancy' | sed 's/.*remark: [^ ]* *//; s/ \[-Rpass.*//' | paste - - - -

@@ -10,7 +10,7 @@ import sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PK = os.path.join(ROOT, "pbrt-v2_amd")
 tag = sys.argv[1] if len(sys.argv) > 1 else "rXX"
-FLAGS = "--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -munsafe-fp-atomics".split()
+FLAGS = "--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops".split()
 ILP = ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]
 TUS = {"hpt_kernels_basic": ILP, "hpt_kernels_basic_i": [], "hpt_kernels_measured": ILP + ["-mllvm", "-greedy-regclass-priority-trumps-globalness=1"], "hpt_kernels_measured_i": [],
        "hpt_kernels_all": [], "hpt_kernels_all_i": [], "hpt_kernels_ext": ILP + ["-mllvm", "-vgpr-regalloc=basic"], "hpt_kernels_ext_i": ["-mllvm", "-vgpr-regalloc=basic"], "hpt_kernels_lean": ILP}   # (= FLAGS_* of pbrt-v2_amd/Makefile, round 5)

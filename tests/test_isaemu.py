@@ -255,3 +255,21 @@ def test_no_shipped_kernel_defines_a_vector_register_above_an_exec_restore():
     objs = gate.device_objects()
     assert len(objs) >= 14          # the ten kernel units + the wavefront pipeline, the device BVH builder, the calibration and exchange kernels
     assert gate.new_sites(objs) == set()
+
+
+PACKED_FP32 = ("v_pk_add_f32", "v_pk_mul_f32", "v_pk_fma_f32")
+
+
+def packed_fp32_in(path):
+    d = gate.disassembly_of(path)
+    return [] if d is None else [line.split("//")[0].strip() for line in d if line.lstrip().startswith(PACKED_FP32)]
+
+
+@needs_build
+def test_no_shipped_kernel_holds_a_packed_fp32_instruction():
+    """the Makefile takes the feature from every HIP unit: some forms of these instructions have given wrong results on the GPU now and then, without an error"""
+    import concurrent.futures
+    objs = gate.device_objects()
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        found = dict(zip(map(os.path.basename, objs), pool.map(packed_fp32_in, objs)))
+    assert not any(found.values()), {k: (len(v), v[0]) for k, v in found.items() if v}
